@@ -208,8 +208,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobArgs a, 
     if (b + W < b1) load(b + W, next);
     const float bm = vecs_max<DT, U>(cur);
     maxima[(b - b0) * 32 + lane] = bm;
-    const bool rise = !(bm <= m);  // NaN rises too, and stays
-    const float nm = rise ? bm : m, mm = nm == -INFINITY ? 0.f : nm;
+    const bool rise = !(bm <= m);  // with NaN too, which the maximum keeps
+    const float nm = max_nan(m, bm), mm = nm == -INFINITY ? 0.f : nm;
     // no further than where f is 0 anyhow, so that a rise from the type's lowest value is no 0 * inf
     const float down = max_nan(m - mm, -1e5f), f = rise ? ex2(down * kLog2e) : 1.0f;
     float2 l2 = make_float2(0.f, 0.f), e2 = l2;

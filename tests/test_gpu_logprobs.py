@@ -113,6 +113,34 @@ def test_rows_without_distribution(env, vocab):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 40, 5), (1, 5000, 32), (1, 151936, 5), (700, 9001, 20)])
+def test_nan_beside_other_logits(env, dtype, rows, vocab, top):
+    """A NaN anywhere, whatever its neighbours and the logits behind it are: NaN numbers, and ids that rank every other logit."""
+    torch, _ = env
+    i = torch.arange(vocab)
+    some = torch.randn(vocab, generator=torch.Generator().manual_seed(vocab))
+    lowest = torch.finfo(getattr(torch, dtype)).min
+    for at in (0, 5, vocab // 2, vocab - 1):
+        one = []
+        for rest in (some, torch.where(i == vocab // 3, 1.0, -math.inf), torch.full((vocab,), -math.inf), torch.where(i < 30, 2.0, lowest)):
+            x = rest.clone()
+            x[at] = math.nan
+            for k in range(1, 4):  # the largest in the same 16 bytes and far away
+                x[(at + k) % vocab], x[(at + 17 * k * k) % vocab] = 40.0 + k, 50.0 - k
+            one += [x, rest.clone()]
+            one[-1][at] = math.nan
+        x = torch.stack(one).to(getattr(torch, dtype))
+        x = x[torch.arange(rows) % len(one)] if rows > 1 else x
+        t = torch.full((len(x),), vocab // 3, dtype=torch.int32, device="cuda")
+        for part in [x] if rows > 1 else x[:, None]:
+            part = part.cuda()
+            got = score(env, part, t[:len(part)], top)
+            check(env, part[:8], t[:min(8, len(part))], top, [g[:8] for g in got])
+            assert np.isnan(got[0]).all() and np.isnan(got[1]).all() and np.isnan(got[3]).all()
+            assert all(np.array_equal(g[k], g[k % 8], equal_nan=True) for g in got for k in range(8, len(part)))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("vocab", [100, 5000, 40000])
 def test_masks_of_the_lowest_value(env, dtype, vocab):
     """A row masked with its type's lowest value is the row masked with -inf, wherever the mask lies: both have weight 0."""
