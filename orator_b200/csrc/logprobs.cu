@@ -14,9 +14,13 @@
 // of its batches in shared memory: the `top` largest logits lie in the few
 // lane batches whose maximum reaches t, the top-th largest of 32 group maxima
 // (`top` different logits reach t), and only those are read again, from L2.
-// Their logits that reach t are placed by counting the larger ones. A row is
-// cut over a cluster of up to 16 CTAs where the rows alone do not fill the GPU;
-// CTA 0 joins the pieces.
+// Their logits that reach t are placed by counting the larger ones. Where too
+// many reach t for that, or fewer than `top` groups have logits at all (masked
+// rows, equal logits), only what lies above t is placed by counting, and the
+// other places go to the first logits that equal t (1,500 bf16 rows of 151,936,
+// 20 places: 111 us; masked but for 3 tokens, with -inf 123, with the type's
+// lowest value 127). A row is cut over a cluster of up to 16 CTAs where the rows
+// alone do not fill the GPU; CTA 0 joins the pieces.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -34,12 +38,20 @@ constexpr int kLpThreads = 256;
 constexpr int kLpCand = 512;      // candidates of a piece that are placed by counting
 constexpr int kLpMaxCluster = 16;
 constexpr int kLpMaxTop = 32;
+constexpr int kLpFew = 256;       // lane batches that are ranked against one another
 
+// Numbers that are in the order of the values (but -0 below +0), and back.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t u) {
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7FFFFFFFu) : ~u);
+}
 // Order of the alternatives: by value (NaN below everything, -0 equal to +0),
 // equal values by index, lowest first. 0 is below every key.
 __device__ __forceinline__ unsigned long long token_key(float v, uint32_t idx) {
-  uint32_t u = v == 0.0f ? 0u : __float_as_uint(v);
-  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  uint32_t u = order_of(v == 0.0f ? 0.0f : v);
   if (v != v) u = 1u;
   return (static_cast<unsigned long long>(u) << 32) | (0xFFFFFFFFu - idx);
 }
@@ -48,8 +60,7 @@ __device__ __forceinline__ uint32_t key_index(unsigned long long k) {
 }
 __device__ __forceinline__ float key_value(unsigned long long k) {
   const uint32_t u = static_cast<uint32_t>(k >> 32);
-  if (u == 1u) return NAN;
-  return __uint_as_float((u & 0x80000000u) ? (u & 0x7FFFFFFFu) : ~u);
+  return u == 1u ? NAN : value_of(u);
 }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -261,16 +272,16 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobArgs a, 
     const unsigned who = __ballot_sync(0xffffffffu, ahead == max(a.top, 1) - 1);
     thr = __shfl_sync(0xffffffffu, mine, who ? __ffs(who) - 1 : 0);
   }
-  if (thr == -INFINITY && a.top > 0) {
-    // Fewer groups than `top` have logits (then each warp has a batch at most): the top-th largest
-    // of the lane batches' maxima.
-    const int n = (b1 - b0) * 32;
+  const int lane_batches = (b1 - b0) * 32;
+  if (thr == -INFINITY && a.top > 0 && lane_batches <= kLpFew) {
+    // Fewer groups than `top` have logits, as in short rows: the top-th largest of the lane
+    // batches' maxima.
     if (t == 0) sm.thr = -INFINITY;
     __syncthreads();
-    for (int i = t; i < n; i += kLpThreads) {
+    for (int i = t; i < lane_batches; i += kLpThreads) {
       const float mine = maxima[i];
       int ahead = 0;
-      for (int j = 0; j < n; ++j) ahead += maxima[j] > mine || (maxima[j] == mine && j < i);
+      for (int j = 0; j < lane_batches; ++j) ahead += maxima[j] > mine || (maxima[j] == mine && j < i);
       if (ahead == a.top - 1) sm.thr = mine;
     }
     __syncthreads();
@@ -278,10 +289,10 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobArgs a, 
   }
   // pm: the piece's maximum; -inf where it has none, NaN where the row has no distribution
   const bool plain = pm > -INFINITY && pm < INFINITY;
+  const bool ordered = pm == pm;  // no NaN
 
   // ---- the lane batches that reach t ----
-  const int lane_batches = (b1 - b0) * 32;
-  if (plain && a.top > 0) {
+  if (ordered && thr > -INFINITY && a.top > 0) {
     for (int i = t; i < lane_batches; i += kLpThreads)
       if (maxima[i] >= thr) {
         const int at = atomicAdd(&sm.listed, 1);
@@ -290,7 +301,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobArgs a, 
   }
   __syncthreads();
   const int listed = min(sm.listed, kLpList);
-  const bool overflow = !plain || sm.listed > kLpList;
+  const bool all_listed = ordered && thr > -INFINITY && sm.listed <= kLpList;
   // Threads of the maximum leave out the batch it came from: it is summed again without it.
   const bool top_thread = m == pm;
   float l = 0.f, pe = 0.f;
@@ -315,8 +326,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobArgs a, 
       }
     }
   }
-  if (a.top > 0 && !overflow) {
-    for (int i = t; i < listed * U; i += kLpThreads) {
+  // The logits of the listed lane batches from `least` on (or above it): candidates.
+  auto gather = [&](int n, float least, bool above) {
+    for (int i = t; i < n * U; i += kLpThreads) {
       const int k = sm.list[i / U];  // vector i % U of lane batch k
       const int v = (b0 + k / 32) * 32 * U + k % 32 + 32 * (i % U);
       if (v >= vecs) continue;
@@ -325,13 +337,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobArgs a, 
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const int idx = v * N + j - lead;
-        if (x[j] >= thr && idx >= 0 && idx < a.vocab) {
+        if (x[j] >= least && !(above && x[j] == least) && idx >= 0 && idx < a.vocab) {
           const int at = atomicAdd(&sm.count, 1);
           if (at < kLpCand) sm.cand[at] = token_key(x[j], idx);
         }
       }
     }
-  }
+  };
+  if (a.top > 0 && all_listed) gather(listed, thr, false);
   l = warp_sum(l);
   pe = warp_sum(pe);
   n = __reduce_add_sync(0xffffffffu, n);
@@ -346,20 +359,109 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobArgs a, 
     out->m = pm, out->l = tl, out->e = te, out->n = tn;
   }
 
+  // Too many logits reach t, or t is -inf: those above t as candidates. Where they are too many
+  // as well, t rises, by halving, to the top-th largest of the lane batches' maxima, so that fewer
+  // than `top` lane batches have anything above it; and then to the top-th largest of those.
+  auto few_above = [&] {
+    for (int stage = 0;; ++stage) {
+      __syncthreads();
+      if (stage < 2) {
+        if (t == 0) sm.listed = 0;
+        __syncthreads();
+        for (int i = t; i < lane_batches; i += kLpThreads)
+          if (maxima[i] > thr) {
+            const int at = atomicAdd(&sm.listed, 1);
+            if (at < kLpList) sm.list[at] = i;
+          }
+      }
+      if (t == 0) sm.count = 0;
+      __syncthreads();
+      const int n = sm.listed;
+      if (n <= kLpList) {
+        gather(n, thr, true);
+        __syncthreads();
+        if (sm.count <= kLpCand) return;
+      }
+      uint32_t lo = order_of(thr), hi = order_of(pm) + 1;  // `top` or more reach lo, not hi
+      while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        const float least = value_of(mid);
+        int reach = 0;
+        if (stage == 0) {
+          for (int i = t; i < lane_batches; i += kLpThreads) reach += maxima[i] >= least;
+        } else {
+          for (int i = t; i < n * U; i += kLpThreads) {
+            const int k = sm.list[i / U];
+            float x[N];
+            unpack16<DT>(load1((b0 + k / 32) * 32 * U + k % 32 + 32 * (i % U)), x);
+#pragma unroll
+            for (int j = 0; j < N; ++j) reach += x[j] >= least;  // above t: in the row
+          }
+        }
+        reach = __reduce_add_sync(0xffffffffu, reach);
+        __syncthreads();
+        if (lane == 0) sm.red_n[warp] = reach;
+        __syncthreads();
+        reach = 0;
+        for (int w = 0; w < W; ++w) reach += sm.red_n[w];
+        (reach >= a.top ? lo : hi) = mid;
+      }
+      thr = value_of(lo);
+    }
+  };
+  // The places behind the candidates: the first logits that equal t, by one warp.
+  auto fill = [&] {
+    int at = sm.count;
+    if (warp > 0) return;
+    for (int b = b0; b < b1 && at < a.top; ++b) {
+      const bool has = maxima[(b - b0) * 32 + lane] >= thr;
+      if (!__any_sync(0xffffffffu, has)) continue;
+#pragma unroll 1
+      for (int u = 0; u < U; ++u) {
+        const int v = b * 32 * U + lane + 32 * u;
+        uint32_t equal = 0;  // a bit for each of the vector's values
+        if (has) {
+          float x[N];
+          unpack16<DT>(load1(v), x);
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const int idx = v * N + j - lead;
+            if (x[j] == thr && idx >= 0 && idx < a.vocab) equal |= 1u << j;
+          }
+        }
+        int mine = __popc(equal), upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += up;
+        }
+        for (int k = at + upto - mine; equal && k < a.top; ++k, equal &= equal - 1)
+          out->keys[k] = token_key(thr, v * N + __ffs(equal) - 1 - lead);
+        at += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+  };
+
   // ---- the piece's largest, in order ----
   if (a.top > 0) {
-    const int count = sm.count;
-    const int c0 = max(0, b0 * 32 * U * N - lead), c1 = min(a.vocab, b1 * 32 * U * N - lead);
-    if (!overflow && count >= min(a.top, c1 - c0) && count <= kLpCand) {
+    auto place = [&] {
+      const int count = sm.count;
       for (int i = t; i < count; i += kLpThreads) {
         const unsigned long long mine = sm.cand[i];
         int ahead = 0;
         for (int j = 0; j < count; ++j) ahead += sm.cand[j] > mine;
         if (ahead < a.top) out->keys[ahead] = mine;
       }
+    };
+    // at least `top` logits reach t, or all that the piece has
+    if (all_listed && sm.count <= kLpCand) {
+      place();
+    } else if (ordered) {
+      few_above();
+      place();
+      fill();
     } else {
-      // no order among the maxima (NaN, +inf, nothing above -inf), or more equal logits than
-      // fit: one pass for each place
+      // no order among the maxima (NaN): one pass for each place
       unsigned long long prev = ~0ull;
       for (int r = 0; r < a.top && prev; ++r) {
         unsigned long long best = 0;

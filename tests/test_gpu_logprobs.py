@@ -159,6 +159,35 @@ def test_masks_of_the_lowest_value(env, dtype, vocab):
     assert (np.abs(lp / torch.finfo(x.dtype).min - 1) <= 2.0**-20).all()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 700, 32), (1, 5000, 5), (1, 30000, 32), (1, 151936, 20), (1, 1 << 19, 32), (600, 40000, 32), (300, 151936, 5)])
+def test_few_legal_tokens(env, dtype, rows, vocab, top):
+    """Rows masked down to some tokens, with -inf or the type's lowest value: the places behind them go to the lowest masked ids."""
+    torch, _ = env
+    tt = getattr(torch, dtype)
+    i = torch.arange(vocab)
+    g = torch.Generator().manual_seed(vocab + top)
+    at = torch.randperm(vocab, generator=g)
+    per = 8 if dtype == "bfloat16" else 4  # values of 16 bytes
+    keeps = [i < 3, i >= vocab - 3, torch.isin(i, at[:3]), torch.isin(i, at[:100]), (i >= vocab // 2) & (i < vocab // 2 + 1000),
+             i % (32 * per) < 8 * per,     # every batch, but a quarter of its lanes
+             i // (128 * per) % 9 == 3, i < 0, i >= 0,
+             (i // (128 * per) == 2) & (i // per % 32 < 31)]  # all values of 31 lanes
+    vals = [2 * torch.randn(vocab, generator=g), torch.randint(0, 3, (vocab,), generator=g).float(), torch.zeros(vocab)]
+    x = torch.stack([torch.where(k, v, mask) for k in keeps for v in vals for mask in (-math.inf, torch.finfo(tt).min)]).to(tt)
+    t = torch.stack([at[0], at[1]] * (len(x) // 2)).int().cuda()
+    if rows == 1:
+        for r in range(len(x)):
+            part = x[r:r + 1].cuda()
+            check(env, part, t[r:r + 1], top, score(env, part, t[r:r + 1], top))
+        return
+    pick = torch.arange(rows) % len(x)
+    part, want = x[pick].cuda(), t[pick.cuda()]
+    got = score(env, part, want, top)
+    check(env, part[:len(x)], t, top, [a[:len(x)] for a in got])
+    assert all(np.array_equal(a[r], a[r % len(x)], equal_nan=True) for a in got for r in range(len(x), rows))
+
+
 def test_sure_rows(env):
     """Entropies far below one keep their digits."""
     torch, _ = env
