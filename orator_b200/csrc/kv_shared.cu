@@ -8,9 +8,8 @@
 // Reference, scales and fp16 operands are the decode kernel's (kv_attention.cu):
 // codes are exact in fp16, K's scale multiplies the score, V's the
 // probability, a row's reference r follows the largest z_j + log2 vs_j and
-// rises only when it is passed by 2^4. Here the bound of a tile, largest z plus
-// largest log2 vs, decides; a tile whose V scales differ by more than 2^12
-// looks at each key's own.
+// rises only when it is passed by 2^4, so that p_j vs_j keeps fp16's digits down
+// to 2^-24 of the row's largest and counts down to 2^-35 of it.
 //
 // One CTA per SM takes an equal share of all (head, 128 rows, 64 keys) tiles in
 // a row; the part of a (head, 128 rows) job that it has is a segment.
@@ -43,12 +42,9 @@ constexpr int kThreads = (kFetchWarp + 4) * 32;  // warpgroups are whole
 constexpr int kSoftRegs = 88, kConvRegs = 56, kRestRegs = 40;
 constexpr int kRaw = 3, kKv = 4;  // stages of raw blocks and of fp16 tiles
 constexpr int kPages = kTile / kPage;
-// p vs is held 2^kUp too large, and a row's reference rises when it is passed by 2^kRoom: at most
-// 2^15. (Two warps rescale their O when one of their 32 rows rises: at a room of 2^8 that is every
-// fourth tile and 17 of 94 us.) The bound of a tile is loose by its V scales' spread, which is at
-// most 2^kWide. What is below 2^-25 2^(kWide - kUp) = 2^-21 of a row's largest p vs is lost, once a
-// key.
-constexpr float kUp = 2.0f, kRoom = 12.0f, kWide = 6.0f;
+// Two warps rescale their O when one of their 32 rows rises. 256 sessions behind 16,384 tokens, the
+// whole call: 122 us with room for 2^4, and 121, 119, 117 and 115 with 2^6, 2^8, 2^10 and 2^12, each
+// of which takes as much off the lower end of p vs; what is lost there is lost once a key.
 constexpr int kColQ = 0, kColS = 64, kColP = 192, kColO = 256;  // S, P, O: one after the other for the teams
 
 template <int D>
@@ -57,7 +53,6 @@ struct SharedSmem {
   alignas(1024) uint8_t v[kKv][kTile * D * 2];
   alignas(128) uint8_t raw[kRaw][kPages * kvq_block_bytes(D)];
   alignas(16) float ks[kKv][kTile], vs[kKv][kTile], ve[kKv][kTile];
-  float ve_max[kKv][2], ve_min[kKv][2];
   int fine[kRaw], kv_fine[kKv];  // bit i: page i is there
   float part[kSlices][kRows], ref[2][kRows];  // what the threads of a row tell one another
   uint64_t raw_full[kRaw], raw_empty[kRaw], kv_full[kKv], kv_empty[kKv];
@@ -323,12 +318,10 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_shared_kernel(KvqCache c, Kvq
           const bool there = fine >> (ct / kPage) & 1;
           const float vs = there ? sc[kPage] : 0.f;
           const float e = fmaxf(
-              __uint_as_float(0x4B000000u | (__float_as_uint(vs) >> 23)) - 8388735.0f, -60.0f);
+              __uint_as_float(0x4B000000u | (__float_as_uint(vs) >> 23)) - 8388735.0f, kLeastV);
           sm.ks[s][ct] = there ? sc[0] : 0.f;
           sm.vs[s][ct] = vs;
           sm.ve[s][ct] = e;
-          const float hi = warp_max(e), lo = -warp_max(-e);
-          if (lane == 0) sm.ve_max[s][ct / 32] = hi, sm.ve_min[s][ct / 32] = lo;
           if (ct == 0) sm.kv_fine[s] = fine;
         }
         // 16 codes at a time, a row by neighbouring lanes, kAtOnce rows at once
@@ -432,12 +425,11 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_shared_kernel(KvqCache c, Kvq
         const float4* ks = reinterpret_cast<const float4*>(&sm.ks[s][part * kKeys]);
         const float4* vs = reinterpret_cast<const float4*>(&sm.vs[s][part * kKeys]);
         const int pos = (seg.t0 + t) * kTile + part * kKeys, fine = sm.kv_fine[s];
-        const float vmax = fmaxf(sm.ve_max[s][0], sm.ve_max[s][1]);
-        const bool wide = vmax - fminf(sm.ve_min[s][0], sm.ve_min[s][1]) > kWide;
+        const float4* ve = reinterpret_cast<const float4*>(&sm.ve[s][part * kKeys]);
         const int there = fine >> (part * kKeys / kPage) & 3;  // of its two pages
         // some row of the warp does not see some key
         const bool edge = pos + kKeys > all_see || there != 3;
-        const float rk = r == -INFINITY ? 0.f : r - kUp;
+        const float rk = r == -INFINITY ? 0.f : r - kLift;
         mbar_sleep(&sm.s_full[team], done & 1, fail);
         fence_after();
         uint32_t x[kKeys];
@@ -464,29 +456,25 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_shared_kernel(KvqCache c, Kvq
             if (2 * j + 1 >= seen || !page) z[j].y = -INFINITY;
           }
         }
-        float top = -INFINITY;
-        if (wide) {
+        float t4[4];
 #pragma unroll
-          for (int j = 0; j < kKeys / 2; ++j)
-            top = fmaxf(top, fmaxf(z[j].x + sm.ve[s][part * kKeys + 2 * j],
-                                   z[j].y + sm.ve[s][part * kKeys + 2 * j + 1]));
-        } else {
-          float t4[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) t4[j] = fmaxf(z[j].x, z[j].y);
-#pragma unroll
-          for (int j = 4; j < kKeys / 2; ++j) t4[j & 3] = max3(t4[j & 3], z[j].x, z[j].y);
-          top = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]) + vmax;
+        for (int j = 0; j < kKeys / 4; ++j) {
+          const float4 e4 = ve[j];
+          const float2 a = add2(z[2 * j], make_float2(e4.x, e4.y)), b = add2(z[2 * j + 1], make_float2(e4.z, e4.w));
+          const int x = 2 * (j & 1);
+          t4[x] = j < 2 ? fmaxf(a.x, a.y) : max3(t4[x], a.x, a.y);
+          t4[x + 1] = j < 2 ? fmaxf(b.x, b.y) : max3(t4[x + 1], b.x, b.y);
         }
+        float top = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]);
         top += rk;  // of z + log2 vs
-        if (pair_barrier_or(pair, top > r + kRoom)) {
+        if (pair_barrier_or(pair, top > r + kSlack)) {
           // ---- some row's reference rises: the rows' maxima, and O where it does ----
           sm.part[slice][row] = top;
           pair_barrier(pair);
           top = fmaxf(top, sm.part[slice ^ 2][row]);
-          const bool rise = top > r + kRoom;
+          const bool rise = top > r + kSlack;
           const float f = rise ? ex2(r - top) : 1.0f;  // 0 for the first
-          const float shift = rise ? rk - (top - kUp) : 0.f;
+          const float shift = rise ? rk - (top - kLift) : 0.f;
 #pragma unroll
           for (int j = 0; j < kKeys / 2; ++j) z[j] = add2(z[j], make_float2(shift, shift));
           if (rise) {
@@ -567,9 +555,9 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_shared_kernel(KvqCache c, Kvq
               make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
       }
       if (slice == 0) {
-        // l and O are both 2^kUp too large
+        // l and O are both 2^kLift too large
         const float sum = (l0 == 0.f ? 0.f : l0 * w0) + (l1 == 0.f ? 0.f : l1 * w1);
-        *reinterpret_cast<float2*>(rec + kRows * D + 2 * row) = make_float2(top - kUp, sum);
+        *reinterpret_cast<float2*>(rec + kRows * D + 2 * row) = make_float2(top - kLift, sum);
         if (row == 0) {
           int* dir = p.directory(a.ws) + 2 * (p.jobs + seg.job);
           if (seg.t0 == 0) dir[0] = blockIdx.x;
