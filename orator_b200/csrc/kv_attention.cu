@@ -241,8 +241,7 @@ struct Piece {
       const float* sc = reinterpret_cast<const float*>((y < 2 ? blk0 : blk1) + 2 * kPage * D);
       ks[y] = sc[g + 8 * (y & 1)];
       vs[y] = sc[kPage + g + 8 * (y & 1)];
-      // floor of log2 vs: its exponent less 127 (2^23 + exponent as a float, less 2^23 + 127)
-      e[y] = fmaxf(__uint_as_float(0x4B000000u | (__float_as_uint(vs[y]) >> 23)) - 8388735.0f, kLeastV);
+      e[y] = scale_exponent(vs[y]);
     }
     uint32_t pb[NT][2 * NP], pl[NT][2 * NP];  // B fragments of P^T, and its second parts
 #pragma unroll

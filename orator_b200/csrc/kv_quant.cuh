@@ -68,6 +68,14 @@ constexpr float kLift = 10.0f;        // p is held 2^10 too large: p vs at most 
 constexpr float kLeastV = -60.0f;     // log2 of V scales counts from here, or r would leave p no range
 constexpr float kLog2e = 1.4426950408889634f;
 
+// What a V scale counts as in a row's reference: floor of its log2 (2^23 + exponent as a float, less
+// 2^23 + 127), kLeastV at least. One that is no number poisons the products, but must not raise the
+// reference, or the sum of probabilities would lose the other keys.
+__device__ __forceinline__ float scale_exponent(float vs) {
+  const float e = __uint_as_float(0x4B000000u | (__float_as_uint(vs) >> 23)) - 8388735.0f;
+  return e > 127.0f ? kLeastV : fmaxf(e, kLeastV);
+}
+
 // Bounded wait that sleeps in the barrier unit (up to a millisecond a try), so
 // that waiting warps take no issue slots from working ones. False after
 // kWaitLimitNs, or at once when another wait already failed.

@@ -317,11 +317,9 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_shared_kernel(KvqCache c, Kvq
           const int fine = sm.fine[rs];
           const bool there = fine >> (ct / kPage) & 1;
           const float vs = there ? sc[kPage] : 0.f;
-          const float e = fmaxf(
-              __uint_as_float(0x4B000000u | (__float_as_uint(vs) >> 23)) - 8388735.0f, kLeastV);
           sm.ks[s][ct] = there ? sc[0] : 0.f;
           sm.vs[s][ct] = vs;
-          sm.ve[s][ct] = e;
+          sm.ve[s][ct] = scale_exponent(vs);
           if (ct == 0) sm.kv_fine[s] = fine;
         }
         // 16 codes at a time, a row by neighbouring lanes, kAtOnce rows at once
