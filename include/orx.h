@@ -226,8 +226,11 @@ typedef struct orx_kvq {
   const int* page_table; /* device [seqs, max_pages]: pool page of positions 16 j .. 16 j + 15 */
   int seqs;              /* up to 65536 */
   int max_pages;         /* up to 2^27 - 1, and seqs * (max_pages + 4) below 2^31 */
-  int* err;              /* device int or NULL: set to 2 where a position, length or page lies
-                            outside the table or the pool (such rows and keys are skipped) */
+  int* err;              /* device int or NULL (nothing is noted), 0 before the first call: set to 2
+                            where a position, length or page lies outside the table or the pool
+                            (such rows and keys are skipped), to 1 where a wait inside
+                            orx_kvq_attention ran out (200 ms): what that call left in out and lse
+                            is not to be used. 1 replaces 2 and stays; no call sets 0 */
 } orx_kvq;
 /* 32 * head_dim + 128 (0 for a head_dim that is not supported). */
 int orx_kvq_block_bytes(int head_dim);

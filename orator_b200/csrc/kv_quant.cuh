@@ -15,8 +15,9 @@
 namespace orx {
 namespace kvq {
 
+// A bad index, which is skipped, does not hide a wait that ran out, after which outputs are missing.
 __device__ __forceinline__ void note_bad(int* err) {
-  if (err) atomicExch(err, kErrBadIndex);
+  if (err) atomicCAS(err, kErrNone, kErrBadIndex);
 }
 
 __device__ __forceinline__ float load_f(const void* p, int dtype, long long i) {
