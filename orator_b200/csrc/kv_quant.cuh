@@ -77,23 +77,35 @@ __device__ __forceinline__ float scale_exponent(float vs) {
   return e > 127.0f ? kLeastV : fmaxf(e, kLeastV);
 }
 
-// Bounded wait that sleeps in the barrier unit (up to a millisecond a try), so
-// that waiting warps take no issue slots from working ones. False after
-// kWaitLimitNs, or at once when another wait already failed.
+// Bounded wait that sleeps in the barrier unit (about 4 us a try, whatever time is asked for), so
+// that waiting warps take no issue slots from working ones. False after kWaitLimitNs, or at once when
+// another wait already failed.
+__device__ __forceinline__ bool mbar_sleep_try(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ uint32_t global_ns_low() {  // 4 s in all
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+  return t;
+}
 __device__ __forceinline__ bool mbar_sleep(uint64_t* bar, uint32_t parity, int* fail) {
-  for (unsigned i = 0; i <= kWaitLimitNs / 1000000; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
-        " selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000)
-        : "memory");
-    if (ok) return true;
+  if (mbar_sleep_try(bar, parity)) return true;
+  const uint32_t t0 = global_ns_low();
+  while (!mbar_sleep_try(bar, parity)) {
     if (*reinterpret_cast<volatile int*>(fail) != 0) return false;
+    if (global_ns_low() - t0 > kWaitLimitNs) {
+      atomicExch(fail, kErrWaitTimeout);
+      return false;
+    }
   }
-  atomicExch(fail, kErrWaitTimeout);
-  return false;
+  return true;
 }
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
