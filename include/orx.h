@@ -216,7 +216,9 @@ int orx_argmax_banned(const float* logits, int n, int ban0, int ban1, int* d_out
  * (fp32), i.e. orx_kvq_block_bytes(head_dim) bytes; value = code * scale, one
  * scale per (token, head). A row with an infinity or a NaN is stored with a
  * NaN scale (what reads it becomes NaN), one whose scale would be below the
- * least normal fp32 number as zeros. */
+ * least normal fp32 number as zeros. In a pool that something else filled, scales
+ * are >= 0 or NaN; e4m3's NaN codes (0x7f, 0xff; never written here) read back as
+ * NaN, and an attention that sees one gives NaN or takes it for 448. */
 typedef struct orx_kvq {
   void* pool;            /* device, 16-byte aligned */
   int pages;             /* pages in the pool (up to 2^27) */

@@ -86,10 +86,9 @@ __device__ __forceinline__ uint32_t quantise4(const float* x, float s, float lo,
 
 // Values of the N codes of w (4 a word) times s, rounded once. int8: the code
 // with its sign bit flipped, as the low byte of 2^23, is 2^23 + 128 + code.
-// e4m3: its bits 6..0 are fp16's bits 13..7 with the exponent bias 8 too low.
+// e4m3: exact in fp16, where its NaN is one too.
 template <int FMT, int N>
 __device__ __forceinline__ void dequantise(const uint32_t* w, float s, float* x) {
-  const float s8 = s * 256.0f;
 #pragma unroll
   for (int i = 0; i < N / 4; ++i) {
     if (FMT == kKvqInt8) {
@@ -99,12 +98,13 @@ __device__ __forceinline__ void dequantise(const uint32_t* w, float s, float* x)
         x[4 * i + j] =
             (__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + j)) - 8388736.0f) * s;
     } else {
+      uint32_t h[2];
+      codes_to_half<FMT>(w[i], h[0], h[1]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint32_t u = __byte_perm(w[i], 0, j ? 0x3424 : 0x1404);  // bytes to the halves' tops
-        const uint32_t h = (u & 0x80008000u) | ((u & 0x7f007f00u) >> 1);
-        x[4 * i + 2 * j] = __half2float(__ushort_as_half(h & 0xffff)) * s8;
-        x[4 * i + 2 * j + 1] = __half2float(__ushort_as_half(h >> 16)) * s8;
+        const float2 f = unpack_half(h[j]);
+        x[4 * i + 2 * j] = f.x * s;
+        x[4 * i + 2 * j + 1] = f.y * s;
       }
     }
   }

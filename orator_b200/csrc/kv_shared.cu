@@ -343,7 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_shared_kernel(KvqCache c, Kvq
             codes_to_half<FMT>(swap ? q.x : q.z, h[4], h[5]);
             codes_to_half<FMT>(swap ? q.y : q.w, h[6], h[7]);
             if (FMT == kKvqE4m3 && kind) {
-              // a slot that was never written may hold a NaN's code, which 0 * would keep
+              // a slot that was never written may hold a NaN's code, which 0 * would keep (and is a key
+              // seen, so that a NaN's code that something else put into the pool counts as 448)
               const __half2 top = __half2half2(__ushort_as_half(0x5F00));  // 448
 #pragma unroll
               for (int z = 0; z < 8; ++z) {
