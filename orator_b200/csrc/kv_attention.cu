@@ -1061,14 +1061,17 @@ Plan attention_plan(const KvqCache& c, int dtype, int q_heads, int q_tokens, int
 }
 
 // CTAs of a job where every job gets a cluster, 0 where the shares are better.
-// Lengths are on the device: max_pages bounds them. A single sequence's jobs
-// are all alike, so nothing is lost to uneven lengths: up to 12 pages a warp
-// (16 heads, 8 kv heads, 128 values: 2,000 tokens 8.4 us here and 11.2 by shares,
-// 8,000 tokens 13.7 and 14.9, 12,000 tokens 16.7 and 15.9). Several sequences:
-// up to 8 (16 of 464 tokens 9.4 and 15.4 us, 100 of 128 tokens 13.2 and 15.1).
-// With shared pages, where the shares read them once for every 8 rows as well
-// and join two parts a row: up to 24 (64 sequences of up to 128 tokens behind
-// 400, 12.3 and 16.4 us, behind 1,024, 16.4 and 27.6; 8 behind 4,800, 15.5 and 14.5).
+// Lengths are on the device: max_pages bounds them. (16 bf16 heads, 8 kv heads,
+// 128 values, int8; us here and by shares.) A single sequence's jobs are all
+// alike, so nothing is lost to uneven lengths: up to 11 pages a warp (2,000
+// tokens 8.2 and 11.2, 10,000 tokens 15.1 and 15.6, 12,000 tokens 16.9 and 16.4).
+// Several sequences: up to 8 (16 of 464 tokens 9.4 and 15.7, 16 of 928 13.4 and
+// 19.2, 100 of 128 13.2 and 15.8). With shared pages, where the shares read them
+// once for every 8 rows as well and join two parts a row: up to 24 (64 sequences
+// of up to 128 tokens behind 1,024, 12 pages a warp, 16.4 and 27.7; 32 behind
+// 4,800, 21 pages, 24.8 and 29.5; 128 behind 2,048, 40 pages, 39.0 and 35.8), but 10
+// where the clusters leave SMs idle, which the shares do not (8 sequences behind
+// 3,200, 8 pages, 13.0 and 13.9; behind 4,800, 11 pages, 15.5 and 14.7).
 int job_ctas(const KvqCache& c, const Plan& p, int shared_pages) {
   const long long jobs = p.joined ? static_cast<long long>(c.kv_heads) * p.group_tiles
                                   : static_cast<long long>(c.seqs) * c.kv_heads * p.job_tiles;
@@ -1080,8 +1083,9 @@ int job_ctas(const KvqCache& c, const Plan& p, int shared_pages) {
   while (ctas < (c.seqs == 1 ? 16 : 8) && ctas * kJobWarps * 2 < pages && jobs * ctas * 2 <= room)
     ctas *= 2;
   const long long each = (pages + ctas * kJobWarps - 1) / (ctas * kJobWarps);  // pages a warp at most
-  if (c.seqs == 1 && !p.joined) return jobs * ctas <= room && each <= 12 ? ctas : 0;
-  return jobs * ctas <= 2 * room && each <= (p.joined ? 24 : 8) ? ctas : 0;
+  if (c.seqs == 1 && !p.joined) return jobs * ctas <= room && each <= 11 ? ctas : 0;
+  const int most = !p.joined ? 8 : jobs * ctas < kCtas ? 10 : 24;
+  return jobs * ctas <= 2 * room && each <= most ? ctas : 0;
 }
 
 template <int D, int FMT, int DT, int NT>
