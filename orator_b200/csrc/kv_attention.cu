@@ -22,7 +22,7 @@ namespace {
 // probability,  p_j = 2^(z_j - r),  l = sum p_j,  O = sum (p_j vs_j) c_j,
 // and the reference r is what the products need: near the largest
 // z_j + log2 vs_j, so that p_j vs_j stays in fp16's range whatever the V scales
-// are (fp32 holds p_j and l in between). A query row is scaled by a power of
+// are, down to 2^-104 (fp32 holds p_j and l in between). A query row is scaled by a power of
 // two to fp16's upper end; fp32 rows and their products are held as two fp16
 // parts (22 bits), bf16 rows' queries are exact in one and their products
 // rounded to one (2^-11). r only rises, and only when a score passes it by

@@ -66,7 +66,10 @@ __device__ __forceinline__ void load_vals(const void* p, long long i, float* x) 
 
 constexpr float kSlack = 4.0f;
 constexpr float kLift = 10.0f;        // p is held 2^10 too large: p vs at most 2^15, down to 2^-35 of it
-constexpr float kLeastV = -60.0f;     // log2 of V scales counts from here, or r would leave p no range
+// log2 of V scales counts from here, or r would leave p no range: p is at most 2^94, and 2^33 of them
+// add up. Products of rows whose scales are all smaller keep fp16's digits down to scales of 2^-104,
+// and count down to 2^-115.
+constexpr float kLeastV = -80.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // What a V scale counts as in a row's reference: floor of its log2 (2^23 + exponent as a float, less
