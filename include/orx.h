@@ -260,7 +260,12 @@ int orx_kvq_attention_workspace(const orx_kvq* c, int q_heads, int q_tokens, int
  * lens: device ints, the sequences' lengths with the query tokens (already
  * written). A row that sees nothing (lens[b] = 0, or t before the first
  * token) gives out = 0 and lse = -inf. lse: [seqs * q_tokens, q_heads] fp32
- * or NULL.
+ * or NULL. q_tokens is at most 4096, seqs * q_tokens * q_heads 2^28, and
+ * seqs * max_pages * kv_heads * (query rows of a kv head) / 8 about 2^41.
+ * Sums and maxima are fp32; products p_j v_j take p_j as one fp16 number for bf16
+ * rows (2^-12 of each) and as two for fp32 rows, and a key whose p_j times V scale
+ * is below 2^-35 of the row's largest may count as none. V rows keep their digits
+ * down to scales of 2^-104.
  * shared (device ints, NULL when shared_pages is 0): the pages of positions
  * [0, 16 * shared_pages) of EVERY sequence, e.g. the head of any table row;
  * they are read once for the whole batch, and the tables' own entries for

@@ -689,6 +689,13 @@ void kvq_heads(const orx::KvqCache& c, int q_heads, int q_tokens, int shared_pag
     throw std::invalid_argument("too many query rows in one call");
   if (shared_pages < 0 || shared_pages > c.max_pages)
     throw std::invalid_argument("shared_pages must be 0 to max_pages");
+  // a share of the work, of 1,628, is counted in 32 bits
+  const long long rows = static_cast<long long>(q_tokens) * (q_heads / c.kv_heads);
+  const long long own = (rows + 7) / 8 * c.seqs, all = (rows * c.seqs + 7) / 8;
+  const long long heads = c.kv_heads, limit = 1ll << 41;
+  if (own * heads > limit / (c.max_pages + 4) || all * heads > limit / (shared_pages + 4) ||
+      own * heads * (c.max_pages + 4) + all * heads * (shared_pages + 4) > limit)
+    throw std::invalid_argument("kv_heads * pages * query rows / 8 must be at most 2^41 in one call");
 }
 }  // namespace
 

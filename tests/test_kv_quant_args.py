@@ -102,6 +102,20 @@ def test_too_many_query_rows():
     refused(ops.KvQuantAttentionWorkspace, cache(seqs=65536), 16, 4096)
 
 
+def test_too_much_work():
+    """Work whose shares could not be counted: 2^41 (page, kv head, 8 query rows) or more, in its own pages or in shared ones."""
+    most = (1 << 27) - 1
+    for c, kw in ((dict(seqs=1, max_pages=most), dict(Hq=512, q_tokens=4096, q_stride=1 << 16, out_stride=1 << 16)),
+                  (dict(seqs=1, max_pages=most, Hkv=1), dict(Hq=1024, q_tokens=256, q_stride=1 << 17, out_stride=1 << 17)),
+                  (dict(seqs=4096, max_pages=500000), dict(Hq=64, q_tokens=1024, q_stride=1 << 13, out_stride=1 << 13, shared=A, shared_pages=400000))):
+        refused(attend, cache(**c), **kw)
+        args = kw["Hq"], kw["q_tokens"], kw.get("shared_pages", 0)
+        refused(ops.KvQuantAttentionWorkspace, cache(**c), *args)
+    for c, args in ((dict(seqs=1, max_pages=most, Hkv=1), (8, 4, 0)), (dict(seqs=1, max_pages=most, Hkv=1), (512, 8, 1000)),
+                    (dict(seqs=65536, max_pages=32000), (8, 1, 0)), (dict(seqs=4096, max_pages=500000), (16, 4, 10))):
+        assert ops.KvQuantAttentionWorkspace(cache(**c), *args) > 0
+
+
 @pytest.mark.parametrize("bad", [dict(logits=0), dict(dtype=2), dict(vocab=0), dict(vocab=-5), dict(vocab=(1 << 19) + 1, row_stride=1 << 20), dict(rows=(1 << 24) + 1), dict(row_stride=99),
                                  dict(top=-1), dict(top=33), dict(vocab=2, top=3), dict(targets=0), dict(top_ids=0),
                                  dict(top_logprobs=0)], ids=str)
