@@ -265,7 +265,8 @@ int orx_kvq_attention_workspace(const orx_kvq* c, int q_heads, int q_tokens, int
  * Sums and maxima are fp32; products p_j v_j take p_j as one fp16 number for bf16
  * rows (2^-12 of each) and as two for fp32 rows, and a key whose p_j times V scale
  * is below 2^-35 of the row's largest may count as none. V rows keep their digits
- * down to scales of 2^-104.
+ * down to scales of 2^-104. Scores beyond 2^22 in size, whose differences fp32 does
+ * not hold, may give rows that are not finite.
  * shared (device ints, NULL when shared_pages is 0): the pages of positions
  * [0, 16 * shared_pages) of EVERY sequence, e.g. the head of any table row;
  * they are read once for the whole batch, and the tables' own entries for

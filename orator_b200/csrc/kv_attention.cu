@@ -265,9 +265,9 @@ struct Piece {
             top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], d));
           // each column by its own scores alone, whatever rows share its tile
           if (top[x] > m[n][x] + kSlack) {
-            const float f = ex2(m[n][x] - top[x]);
+            const float h = ex2_half(m[n][x] - top[x]), f = h * h;
             m[n][x] = top[x];
-            l[n][x] *= f;
+            l[n][x] = l[n][x] * h * h;
 #pragma unroll
             for (int w = 0; w < 2 * kW; ++w) {
               o[n][w][x] *= f;
@@ -374,8 +374,8 @@ template <int E>
 __device__ __forceinline__ void join_into(float& m, float& l, float* o, float bm, float bl,
                                           const float* bo) {
   if (bl == 0.f) return;
-  const float nm = fmaxf(m, bm), f = ex2(m - nm), bf = ex2(bm - nm);
-  l = l * f + bl * bf;
+  const float nm = fmaxf(m, bm), h = ex2_half(m - nm), bh = ex2_half(bm - nm), f = h * h, bf = bh * bh;
+  l = l * h * h + bl * bh * bh;
 #pragma unroll
   for (int x = 0; x < E; ++x) o[x] = o[x] * f + bo[x] * bf;
   m = nm;
@@ -822,8 +822,8 @@ __global__ void __launch_bounds__(kSplit > kJoinWarps ? 1024 : kJoinWarps * 32)
 #pragma unroll
     for (int w = 0; w < kSplit; ++w) {
       if (sh_l[w] == 0.f) continue;
-      const float f = ex2(sh_m[w] - m);
-      l += sh_l[w] * f;
+      const float h = ex2_half(sh_m[w] - m), f = h * h;
+      l += sh_l[w] * h * h;
 #pragma unroll
       for (int y = 0; y < E; ++y) o[y] += sh_o[w][lane * E + y] * f;
     }

@@ -220,6 +220,9 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// 2^(d / 2), d <= 0: sums of probabilities are scaled by 2^d in two steps, as they may be large and 2^d
+// too small for a number where the V scales are far apart.
+__device__ __forceinline__ float ex2_half(float d) { return ex2(0.5f * d); }
 // ln(l 2^r): the exponent of l goes to r first, as the two may be far apart.
 __device__ __forceinline__ float ln_sum(float r, float l) {
   if (!(l < INFINITY)) return l + r;

@@ -472,13 +472,13 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_shared_kernel(KvqCache c, Kvq
           pair_barrier(pair);
           top = fmaxf(top, sm.part[slice ^ 2][row]);
           const bool rise = top > r + kSlack;
-          const float f = rise ? ex2(r - top) : 1.0f;  // 0 for the first
+          const float h = rise ? ex2_half(r - top) : 1.0f, f = h * h;  // 0 for the first
           const float shift = rise ? rk - (top - kLift) : 0.f;
 #pragma unroll
           for (int j = 0; j < kKeys / 2; ++j) z[j] = add2(z[j], make_float2(shift, shift));
           if (rise) {
             r = top;
-            l *= f;
+            l = l * h * h;
           }
           if (t > 1) {
             mbar_sleep(&sm.o_done[team], (done - 1) & 1, fail);
@@ -535,7 +535,8 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_shared_kernel(KvqCache c, Kvq
       fence_after();
       const float r0 = sm.ref[0][row], r1 = sm.ref[1][row], top = fmaxf(r0, r1);
       const float l0 = sm.part[0][row] + sm.part[2][row], l1 = sm.part[1][row] + sm.part[3][row];
-      const float w0 = l0 == 0.f ? 0.f : ex2(r0 - top), w1 = l1 == 0.f ? 0.f : ex2(r1 - top);
+      const float h0 = l0 == 0.f ? 0.f : ex2_half(r0 - top), h1 = l1 == 0.f ? 0.f : ex2_half(r1 - top);
+      const float w0 = h0 * h0, w1 = h1 * h1;
       float* rec = p.tc_records(a.ws, D) +
                    static_cast<long long>(blockIdx.x + seg.job) * kRows * (D + 4);
 #pragma unroll 1
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_shared_kernel(KvqCache c, Kvq
       }
       if (slice == 0) {
         // l and O are both 2^kLift too large
-        const float sum = (l0 == 0.f ? 0.f : l0 * w0) + (l1 == 0.f ? 0.f : l1 * w1);
+        const float sum = (l0 == 0.f ? 0.f : l0 * h0 * h0) + (l1 == 0.f ? 0.f : l1 * h1 * h1);
         *reinterpret_cast<float2*>(rec + kRows * D + 2 * row) = make_float2(top - kLift, sum);
         if (row == 0) {
           int* dir = p.directory(a.ws) + 2 * (p.jobs + seg.job);
